@@ -149,8 +149,10 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits``: 32, or 8 for moments in 8 bits (2 bytes a parameter).  ``master``: keep fp32 master weights
     of bf16 and fp16 parameters (default: yes).  ``seed``: of the 8-bit rounding.  Parameters are contiguous GPU
-    tensors.  A step can be captured into a graph once every parameter has its state (after one eager step);
-    the learning rate and the other numbers are those of the capture then, the step count goes on."""
+    tensors.  A step can be captured into a graph after one eager step with the same parameters' gradients, which
+    gives each its state and those that go together their count; the learning rate and the other numbers are those of
+    the capture then, the step count goes on, and the graph keeps to the state's tensors as they were captured (an
+    eager step of fewer parameters, or a loaded state, puts others in their place)."""
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, master: bool = True, seed: int = 0):
@@ -209,6 +211,10 @@ class AdamW(torch.optim.Optimizer):
                 members = [p for k in kinds for p in cohorts[step_id, k]]
                 step = self.state[members[0]]["step"]
                 if holders.get(step_id, len(members)) > len(members):     # the others stay where they are
+                    if step.is_cuda and torch.cuda.is_current_stream_capturing():
+                        # each replay would copy the count that stays, and stand still
+                        raise RuntimeError("AdamW: a captured step of some of the parameters that have been stepped "
+                                           "together; run one eager step with these gradients first")
                     step = step.clone()
                     for p in members:
                         self.state[p]["step"] = step

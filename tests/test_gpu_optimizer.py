@@ -1,0 +1,57 @@
+"""AdamW on the GPU: captured steps of a part of the parameters."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_of_a_part(pkg, bits):
+    """Parameters a and b have been stepped together; a step of a alone gives a its own count.  Captured, that would be
+    copied from the common one at each replay and never go on: it is refused, and after one such eager step a captured
+    one counts on as eager steps do."""
+    gen = torch.Generator(device=DEV).manual_seed(bits)
+    start, grad = (torch.randn(300, 40, generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+    runs = []
+    for captured in (False, True):
+        a, b = (torch.nn.Parameter(start.clone()) for _ in range(2))
+        opt = pkg.AdamW([a, b], lr=1e-2, state_bits=bits)
+        a.grad, b.grad = grad.clone(), grad.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            opt.step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        b.grad = None
+        if captured:
+            counts = [opt.state[p]["step"] for p in (a, b)]
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                with pytest.raises(RuntimeError, match="eager"):
+                    opt.step()
+                start.clone()                               # a capture of nothing else would warn
+            assert all(opt.state[p]["step"] is c for p, c in zip((a, b), counts))
+            assert [int(c) for c in counts] == [1, 1]
+            del graph
+        opt.step()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
+        seen = []
+        for rep in range(3):
+            graph.replay() if captured else opt.step()
+            torch.cuda.synchronize()
+            s = opt.state[a]
+            second = "exp_avg_sq" if bits == 32 else "exp_avg_sq_root"
+            seen.append([t.clone() for t in (a.detach(), s["master"], s["exp_avg"].float(), s[second].float(), s["step"])])
+            (start * 2).sum().item()                        # eager work between the replays
+        assert [int(s[-1]) for s in seen] == [3, 4, 5] and int(opt.state[b]["step"]) == 1
+        runs.append(seen)
+    for x, y in zip(*runs):
+        assert all(torch.equal(s, t) for s, t in zip(x, y))
