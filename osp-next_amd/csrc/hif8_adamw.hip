@@ -194,7 +194,7 @@ template <int DT, bool BITS8, bool MASTER> __global__ __launch_bounds__(kThreads
     for (int k = 0; k < 8; ++k) {
         m[k] = m[k] * A.b1 + g[k] * A.one_b1;
         v[k] = v[k] * A.b2 + g[k] * g[k] * A.one_b2;
-        r[k] = __fsqrt_rn(v[k]);
+        r[k] = __builtin_sqrtf(v[k]);       // to nearest; __fsqrt_rn is the instruction alone, off by one in the last place
         p[k] = p[k] * A.keep - m[k] / (r[k] * co.root + A.eps) * co.step_size;
     }
     if (MASTER) write8<HIF8_DTYPE_F32>(T.master, i, left, p);

@@ -1,6 +1,7 @@
-"""AdamW on the GPU: captured steps of a part of the parameters."""
+"""AdamW on the GPU: captured steps of a part of the parameters, the root's last bit."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -55,3 +56,20 @@ def test_captured_step_of_a_part(pkg, bits):
         runs.append(seen)
     for x, y in zip(*runs):
         assert all(torch.equal(s, t) for s, t in zip(x, y))
+
+
+def test_root_is_rounded_correctly(pkg):
+    """m = 1, v given, no decay, p = 0, lr = 1, eps = 0 and corrections of 1 (1 - 2^-201): p = -1 / sqrt(v), the root
+    and the quotient each rounded to nearest, as numpy rounds them."""
+    n = 1 << 20
+    rng = np.random.default_rng(7)
+    v = np.exp2(rng.uniform(-120.0, 120.0, n)).astype(np.float32)
+    v[:64] = np.float32(2.0) ** -149 * np.arange(1, 65, dtype=np.float32)          # subnormal numbers
+    want = -(np.float32(1.0) / np.sqrt(v))
+    p, g, m = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), torch.full((n,), 2.0, device=DEV)
+    vt = torch.from_numpy(v * np.float32(2.0)).to(DEV)
+    pkg.adamw_step([p], [g], [m], [vt], torch.full((1,), 200, dtype=torch.int64, device=DEV), lr=1.0, betas=(0.5, 0.5),
+                   eps=0.0, weight_decay=0.0)
+    assert (m == 1).all() and np.array_equal(vt.cpu().numpy(), v)
+    wrong = int((p.cpu().numpy() != want).sum())
+    assert wrong == 0, f"{wrong} of {n}"
