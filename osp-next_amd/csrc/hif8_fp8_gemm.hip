@@ -127,8 +127,10 @@ __global__ __launch_bounds__(kThreads, W * NST > 4 ? 1 : 2) void k_fp8_gemm(cons
     // scale bytes: 16 of each row (16 k steps) in one of two windows
     constexpr uint32_t kScales = kStage * NST, kWindow = 2 * uint32_t(T) * 16;
     constexpr int LS = (2 * T + 255) / 256;      // loads of a wave and window, 64 rows each
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kScales + 2 * kWindow];
-    __shared__ float bias[T];
+    // The one array of the kernel, so that it begins at LDS address 0: loads into LDS address from there.
+    constexpr uint32_t kBias = kScales + 2 * kWindow;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kBias + T * sizeof(float)];
+    float *bias = (float *)(smem + kBias);
     ASMV("; lds base %0" ::"v"(uint32_t(uintptr_t(smem))) : "memory");
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t r = lane & 31u, h = lane >> 5;
@@ -411,7 +413,7 @@ __global__ __launch_bounds__(kThreads, W * NST > 4 ? 1 : 2) void k_fp8_gemm(cons
         constexpr int dt = decltype(tag)::value;
         constexpr uint32_t kSize = dt == HIF8_DTYPE_F32 ? 4 : 2, kLanes = 32 * W * kSize / 16, kRows = 64 / kLanes;
         constexpr uint32_t kPitch = 32 * W * kSize + 16, kPart = 32 * kPitch;
-        static_assert(4 * 2 * kPart <= kScales + 2 * kWindow, "the outputs fit");
+        static_assert(4 * 2 * kPart <= kBias, "the outputs fit");
         const uint32_t row_bytes = uint32_t(A.N) * kSize;
         uint8_t *to = out + m0 * int64_t(row_bytes);
         const bool vec = row_bytes % 16 == 0;
