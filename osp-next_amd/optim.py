@@ -24,6 +24,7 @@ from torch import Tensor
 from . import _lib
 
 BLOCK = 128
+MOST = 1 << 34                # elements of a tensor
 Moment = Union[Tensor, Tuple[Tensor, Tensor]]
 
 
@@ -105,9 +106,29 @@ def _rows(params, grads, exp_avgs, exp_avg_sqs, masters):
             g = g.contiguous()
             keep.append(g)
         by_dtype.setdefault(dt, []).append((pp, g.data_ptr(), mp, vp, ms, vs, wp, count, i))
+    if len(by_dtype) > 1:
+        _check_types(by_dtype, bits8)
     if dev.type != "cuda":
         raise ValueError(f"adamw_step takes GPU tensors (there is no CPU route), got {dev}")
     return bits8, by_dtype, keep
+
+
+def _check_types(by_dtype: dict, bits8: bool) -> None:
+    """What the entry point refuses, for a step of several types: it looks at one type's tensors, and none may be
+    refused once another type's call has been made."""
+    spans = []
+    for dt, rows in by_dtype.items():
+        t = np.array(rows, dtype=np.int64)
+        n, moment = t[:, 7], 1 if bits8 else 4
+        if (n > MOST).any():
+            raise ValueError(f"adamw_step: a tensor of {n.max()} elements (at most {MOST})")
+        for at, size in ((0, dt.itemsize * n), (2, moment * n), (3, moment * n), (4, (n + BLOCK - 1) // BLOCK),
+                         (5, (n + BLOCK - 1) // BLOCK), (6, 4 * n)):
+            spans.append(np.stack((t[:, at], t[:, at] + size), 1)[t[:, at] != 0])
+    s = np.concatenate(spans)
+    s = s[np.argsort(s[:, 0])]
+    if (s[1:, 0] < s[:-1, 1]).any():
+        raise ValueError("adamw_step: two tensors that it writes share memory")
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Moment],
