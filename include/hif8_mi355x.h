@@ -614,7 +614,8 @@ int hif8_layer_norm_bwd(const void *dy, const void *x, int dtype, int64_t rows, 
  * element's place decide, and a positive one never to zero.
  * step (device) holds the steps done; advance: t = *step + 1, and *step becomes t; otherwise t = *step (the
  * further calls of a step that takes several).  tensors is host memory, read before the call returns;
- * workspace is hif8_adamw_workspace_bytes() of device memory.  No two written tensors may overlap (HIF8_ERR_ARG).
+ * workspace is hif8_adamw_workspace_bytes() of device memory.  No two written tensors may overlap, and no gradient
+ * a written tensor (HIF8_ERR_ARG); gradients may overlap each other.
  */
 typedef struct {
     void *param;

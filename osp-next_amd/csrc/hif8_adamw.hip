@@ -225,11 +225,12 @@ template <int DT, bool BITS8, bool MASTER> __global__ __launch_bounds__(kThreads
     }
 }
 
-// Whether no two of the tensors that a call writes share a byte.
+// Whether no two of the tensors that a call writes share a byte, and no gradient one with any of them.
 bool apart(const hif8_adamw_tensor *t, int64_t count, int64_t size, bool bits8)
 {
-    std::vector<std::pair<uint64_t, uint64_t>> r;
-    r.reserve(size_t(count) * 5);
+    typedef std::pair<uint64_t, uint64_t> Span;
+    std::vector<Span> r;
+    r.reserve(size_t(count) * 6);
     auto add = [&](const void *p, int64_t bytes) {
         if (p) r.emplace_back(uint64_t(p), uint64_t(p) + uint64_t(bytes));
     };
@@ -247,6 +248,12 @@ bool apart(const hif8_adamw_tensor *t, int64_t count, int64_t size, bool bits8)
     std::sort(r.begin(), r.end());
     for (size_t k = 1; k < r.size(); ++k)
         if (r[k].first < r[k - 1].second) return false;
+    for (int64_t k = 0; k < count; ++k) {
+        const uint64_t g0 = uint64_t(t[k].grad), g1 = g0 + uint64_t(t[k].n * size);
+        // the last written tensor that begins before the gradient's end
+        const auto at = std::lower_bound(r.begin(), r.end(), Span{g1, 0});
+        if (at != r.begin() && (at - 1)->second > g0) return false;
+    }
     return true;
 }
 

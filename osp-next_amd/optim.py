@@ -116,7 +116,7 @@ def _rows(params, grads, exp_avgs, exp_avg_sqs, masters):
 def _check_types(by_dtype: dict, bits8: bool) -> None:
     """What the entry point refuses, for a step of several types: it looks at one type's tensors, and none may be
     refused once another type's call has been made."""
-    spans = []
+    spans, grads = [], []
     for dt, rows in by_dtype.items():
         t = np.array(rows, dtype=np.int64)
         n, moment = t[:, 7], 1 if bits8 else 4
@@ -125,17 +125,22 @@ def _check_types(by_dtype: dict, bits8: bool) -> None:
         for at, size in ((0, dt.itemsize * n), (2, moment * n), (3, moment * n), (4, (n + BLOCK - 1) // BLOCK),
                          (5, (n + BLOCK - 1) // BLOCK), (6, 4 * n)):
             spans.append(np.stack((t[:, at], t[:, at] + size), 1)[t[:, at] != 0])
-    s = np.concatenate(spans)
+        grads.append(np.stack((t[:, 1], t[:, 1] + dt.itemsize * n), 1))
+    s, g = np.concatenate(spans), np.concatenate(grads)
     s = s[np.argsort(s[:, 0])]
     if (s[1:, 0] < s[:-1, 1]).any():
         raise ValueError("adamw_step: two tensors that it writes share memory")
+    before = np.searchsorted(s[:, 0], g[:, 1]) - 1          # the last written tensor that begins before the gradient's end
+    if (s[before, 1] > g[:, 0])[before >= 0].any():
+        raise ValueError("adamw_step: a gradient shares memory with a tensor that it writes")
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Moment],
                exp_avg_sqs: Sequence[Moment], step: Tensor, *, lr: float, betas: Tuple[float, float] = (0.9, 0.999),
                eps: float = 1e-8, weight_decay: float = 0.01, masters: Optional[Sequence[Tensor]] = None,
                seed: int = 0) -> None:
-    """One AdamW step in place on contiguous bf16, fp16 or fp32 parameters, gradients of their types.
+    """One AdamW step in place on contiguous bf16, fp16 or fp32 parameters, gradients of their types.  No two tensors that
+    it writes may share memory, nor a gradient with one of them.
 
     ``exp_avgs`` and ``exp_avg_sqs`` are fp32 tensors, or (codes, scales) pairs in 8 bits, of m and of sqrt(v)
     (``pack_moment``).  ``masters``: fp32 master weights of 16-bit parameters.  ``step``: an int64 tensor of one

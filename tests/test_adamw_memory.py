@@ -51,9 +51,34 @@ def test_a_later_types_tensor_too_long(pkg):
     from ospnext_amd import optim
 
     def at(k, n):
-        return (k, k, k + (1 << 40), k + (1 << 41), 0, 0, 0, n, 0)
+        return (k, k + (1 << 39), k + (1 << 40), k + (1 << 41), 0, 0, 0, n, 0)
     rows = {torch.float32: [at(1 << 44, 64)], torch.bfloat16: [at(1 << 45, 1 << 34)]}
     optim._check_types(rows, False)
     rows[torch.bfloat16] = [at(1 << 45, (1 << 34) + 1)]
     with pytest.raises(ValueError, match="elements"):
         optim._check_types(rows, False)
+
+
+def test_gradients(pkg):
+    """A gradient may be shared by parameters, but not be what the step writes."""
+    import numpy as np
+    L = pkg._lib.load()
+    at = 0x1000000                                          # never dereferenced: every call is refused
+
+    def step(rows):
+        t = np.array(rows, dtype=np.uint64)
+        return L.hif8_adamw_step(t.ctypes.data, len(rows), 1, 32, at, 1, 1e-3, 0.9, 0.99, 1e-8, 0.0, 0, at, 64, None)
+
+    def one(p, g, n=64):
+        return (p, g, p + 0x1000, p + 0x2000, 0, 0, 0, n, 0)
+    p, q, g = at + 0x10000, at + 0x20000, at + 0x30000
+    assert step([one(p, p)]) == -1                          # its own parameter
+    assert step([one(p, g), one(q, p + 252)]) == -1         # another's last element
+    assert step([one(p, p + 0x1000 - 252)]) == -1           # the first of a moment
+    assert step([one(p, g), one(q, q + 0x2080)]) == -1      # inside the other moment
+    f32 = torch.float32
+    shared = torch.zeros(64)
+    with pytest.raises(ValueError, match="gradient"):       # across types
+        call(pkg, row(64, f32, g=shared), row(64, torch.bfloat16, m=shared))
+    with pytest.raises(ValueError, match="GPU"):            # of two parameters
+        call(pkg, row(64, f32, g=shared), row(64, f32, g=shared), row(8, torch.bfloat16))
