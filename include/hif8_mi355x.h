@@ -590,7 +590,7 @@ int hif8_fp8_linear_bwd(const void *g, int g_dtype, int64_t ld_g, int g_format, 
  * weight (w, or w - 1 with plus_one: a modulation's scale) and bias are of weight_dtype, one row of dim values
  * per group at a stride of ld_weight elements; rows / groups consecutive rows of x make a group.  NULL: 1 (or 0
  * for the bias).  stats [rows][2] fp32 takes mean and rstd for the backward pass (NULL: not kept), 8-byte aligned.
- * dim at most 8192 (HIF8_ERR_SHAPE).
+ * dim at most 8192, groups at most 65535 (HIF8_ERR_SHAPE).
  */
 int hif8_layer_norm_fwd(const void *x, int dtype, int64_t rows, int64_t dim, int64_t groups, const void *weight,
                         const void *bias, int weight_dtype, int64_t ld_weight, int plus_one, float eps, void *y,

@@ -230,6 +230,9 @@ def grouped_weight(layers) -> Optional[GroupedWeight]:
 # ------------------------------------------------------------- with gradients
 
 
+MAX_GROUPS = 65535            # of the entry points: a grid's second dimension
+
+
 class _LayerNormFunction(torch.autograd.Function):
     """y = norm(x) * w + b over x's last dim; weight and bias hold ``groups`` rows of D (in any shape, with one
     row stride) or are None; ``plus``: w = 1 + weight."""
@@ -337,7 +340,7 @@ def modulated_layer_norm(x: Tensor, shift: Optional[Tensor] = None, scale: Optio
     """``norm(x) * (1 + scale) + shift`` (osp_next.py:941, :954) with gradients for x, shift and scale, in fp32
     arithmetic and rounded once to x's dtype.  ``shift`` and ``scale`` are [D], or [B, 1, D] (as many ones as x
     has dims between) for x [B, ..., D], rows of a larger tensor included; their gradients are summed in fp32
-    over a batch entry's rows."""
+    over a batch entry's rows.  More than 65535 entries are done in parts, which are put together by a copy."""
     D = _norm_rows(x, (("shift", shift), ("scale", scale)), eps)
     counts = [1, 1]
     for i, (name, t) in enumerate((("shift", shift), ("scale", scale))):
@@ -351,4 +354,7 @@ def modulated_layer_norm(x: Tensor, shift: Optional[Tensor] = None, scale: Optio
     if groups > 1:       # one for all entries beside one for each: a row for each, whose gradients torch adds up
         shift, scale = (t if t is None or n == groups else t.reshape(1, D).expand(groups, D)
                         for t, n in zip((shift, scale), counts))
+    if groups > MAX_GROUPS:
+        parts = zip(*((None,) * -(-groups // MAX_GROUPS) if t is None else t.split(MAX_GROUPS) for t in (x, shift, scale)))
+        return torch.cat([modulated_layer_norm(*part, eps) for part in parts])
     return _LayerNormFunction.apply(x, scale, shift, float(eps), True, groups)
