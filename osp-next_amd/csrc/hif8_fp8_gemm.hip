@@ -498,13 +498,15 @@ struct Choice {
     int tile, splits;
 };
 // The plan that takes the least time by what the tiles were measured to take: a step of 128 k and the rest of a
-// tile in microseconds, with one workgroup a CU and with as many as fit (256 CUs), and for k ranges a launch and
-// 8 bytes of memory traffic a partial sum.  Each tile size has its place (M x N x K, microseconds with tiles of
-// 256 / 128 / 64): 5120 x 5120 x 8192 200 / 214 / 333, 4680 x 1536 x 8960 86 / 63 / 113, 128 x 5120 x 5120
-// 50 / 21 / 16; and so have ranges: 1536 x 1536 x 32760 in 7 of 256-wide tiles 85, unsplit 285; 256 x 1536 x 8960 in
-// 6 of 128 17, unsplit 31; 16 x 13824 x 5120 in 2 of 64 18, unsplit 15.  A 128-wide tile alone on its CU waits for its
-// loads with two stages: with three 512 x 5120 x 5120 takes 22, with two 36; where two tiles fit a CU each fills the
-// other's waits, and 4680 x 1536 x 8960 takes 63 with two stages and 73 with three.  Four are no better than three.
+// tile in microseconds, with one workgroup a CU and with as many as fit (256 CUs), and for k ranges a launch, a read
+// after the other of each range's sums and 8 bytes of memory traffic a partial sum.  Each tile size has its place (M x
+// N x K, microseconds with tiles of 256 / 128 / 64): 5120 x 5120 x 8192 191 / 215 / 333, 4680 x 1536 x 8960 87 / 63 /
+// 105, 128 x 5120 x 5120 50 / 19 / 13; and so have ranges: 1536 x 1536 x 32760 in 7 of 256-wide tiles 84, unsplit 285;
+// 16 x 1536 x 8960 in 7 of 64 11, in 14 15, unsplit 18; but 16 x 13824 x 5120 in 2 of 64 17, unsplit 14, and 128 x 5120 x
+// 5120 in 3 15.  A 128-wide tile alone on its CU waits for its loads with two stages: with three 512 x 5120 x 5120 takes
+// 21, with two 32; where two tiles fit a CU each fills the other's waits, and 4680 x 1536 x 8960 takes 63 with two
+// stages and 69 with three.  Four are no better than three.  Over 130 products of 1 to 8960 rows the plan taken is within
+// 10 % of the best of all plans, 0.5 % on average.
 Choice choose(int64_t M, int64_t N, int64_t nk)
 {
     struct Tile {
@@ -513,7 +515,7 @@ Choice choose(int64_t M, int64_t N, int64_t nk)
         double step, full_step, rest;
     };
     constexpr Tile kinds[] = {{kBig, 256, 256, 1.15, 1.15, 7.0}, {kMid, 128, 512, 0.8, 0.95, 3.0}, {kDeep, 128, 256, 0.46, 0.46, 3.0},
-                              {kSmall, 64, 512, 0.38, 0.45, 2.0}};
+                              {kSmall, 64, 512, 0.22, 0.48, 2.0}};
     Choice best{kBig, 256, 1};
     double least = 1e300;
     for (const Tile &t : kinds) {
@@ -521,7 +523,7 @@ Choice choose(int64_t M, int64_t N, int64_t nk)
         for (int64_t s = 1; s <= 16 && (s == 1 || (nk >= 4 * s && tiles * s <= t.room)); ++s) {
             const int64_t steps = (nk + s - 1) / s, rounds = (tiles * s + t.room - 1) / t.room;
             double us = double(rounds) * (double(steps) * (tiles * s <= 256 ? t.step : t.full_step) + t.rest);
-            if (s > 1) us = 1.05 * (us + 4.0 + double(s) * double(M) * double(N) * 8.0 / 4e6);
+            if (s > 1) us = 1.05 * (us + 3.5 + double(s) * (0.25 + double(M) * double(N) * 8.0 / 4e6));
             if (us < least) {
                 least = us;
                 best = Choice{t.plan, t.size, int(s)};
