@@ -182,15 +182,19 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, master: bool = True, seed: int = 0):
-        if isinstance(lr, Tensor):
-            raise TypeError("lr is a number")
-        if not lr >= 0 or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"AdamW: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits is 8 or 32, got {state_bits}")
         self.seed = int(seed)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master=master))
+
+    def add_param_group(self, param_group: dict) -> None:
+        g = {**self.defaults, **param_group}
+        if isinstance(g["lr"], Tensor):
+            raise TypeError("lr is a number")
+        if not g["lr"] >= 0 or not g["eps"] >= 0 or not g["weight_decay"] >= 0 or not all(0 <= b < 1 for b in g["betas"]):
+            raise ValueError("AdamW: " + ", ".join(f"{k} {g[k]}" for k in ("lr", "betas", "eps", "weight_decay")))
+        if g["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32, got {g['state_bits']}")
+        super().add_param_group(param_group)
 
     def _new_state(self, p: Tensor, group: dict, step: Tensor) -> dict:
         s = dict(step=step)
