@@ -35,11 +35,11 @@ def pack_moment(t: Tensor) -> Tuple[Tensor, Tensor]:
         raise ValueError("pack_moment takes a contiguous tensor")
     from .fp8 import fp8_quantize
     n = t.numel()
-    rows = (n + BLOCK - 1) // BLOCK
-    flat = torch.zeros(rows * BLOCK, dtype=torch.float32, device=t.device)
+    row = 64 * BLOCK              # 64 blocks a row, so that 2^34 elements stay within the rows that the quantiser takes
+    flat = torch.zeros(max(1, (n + row - 1) // row) * row, dtype=torch.float32, device=t.device)
     flat[:n] = t.detach().reshape(-1)
-    q = fp8_quantize(flat.view(rows, BLOCK))
-    return q.codes.view(-1)[:n].clone().view(t.shape), q.scales[:, 0].contiguous()
+    q = fp8_quantize(flat.view(-1, row))
+    return q.codes.view(-1)[:n].clone().view(t.shape), q.scales.view(-1)[:(n + BLOCK - 1) // BLOCK].clone()
 
 
 def unpack_moment(moment: Tuple[Tensor, Tensor]) -> Tensor:
