@@ -611,7 +611,8 @@ int hif8_layer_norm_bwd(const void *dy, const void *x, int dtype, int64_t rows, 
  * weight and param takes its rounding.  state_bits 32: exp_avg and exp_avg_sq are fp32 m and v.  8: e4m3 codes of
  * m and of sqrt(v), with a scale byte for each 128 elements in *_scales (ceil(n / 128) bytes); sqrt(v) is
  * rounded up with the probability of its fraction, by a number that seed, t, the tensor's index and the
- * element's place decide, and a positive one never to zero.
+ * element's place decide, and a positive one never to zero.  A block with an infinity
+ * or NaN becomes NaN.
  * step (device) holds the steps done; advance: t = *step + 1, and *step becomes t; otherwise t = *step (the
  * further calls of a step that takes several).  tensors is host memory, read before the call returns;
  * workspace is hif8_adamw_workspace_bytes() of device memory.  No two written tensors may overlap, and no gradient

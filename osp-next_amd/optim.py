@@ -8,7 +8,9 @@ A step with t - 1 steps before it::
 With 8-bit moments, m and sqrt(v) are e4m3 codes with a power-of-two scale for each 128 elements: 2 bytes a
 parameter in place of 8.  sqrt(v) is rounded up or down at random (by numbers that the seed, the step and the
 element decide, so that a run can be repeated): b2 near 1 moves it by less than half a step of its code,
-and rounded to nearest it would never move.  bf16 and fp16 parameters may have fp32 master weights, which
+and rounded to nearest it would never move.  A scale is finite: one gradient that is infinite or NaN makes its
+block's 128 moments NaN, and with the next step their parameters, where fp32 moments lose its own alone; look
+for such gradients before the step.  bf16 and fp16 parameters may have fp32 master weights, which
 take the update, the parameter being their rounding.
 
 The step count is on the GPU and every launch goes by it, so that a captured step counts on with each replay.

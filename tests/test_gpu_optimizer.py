@@ -1,4 +1,4 @@
-"""AdamW on the GPU: captured steps of a part of the parameters, the root's last bit."""
+"""AdamW on the GPU: captured steps of a part of the parameters, the root's last bit, gradients that are not finite."""
 from __future__ import annotations
 
 import numpy as np
@@ -73,3 +73,24 @@ def test_root_is_rounded_correctly(pkg):
     assert (m == 1).all() and np.array_equal(vt.cpu().numpy(), v)
     wrong = int((p.cpu().numpy() != want).sum())
     assert wrong == 0, f"{wrong} of {n}"
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradient_that_is_not_finite(pkg, bits, bad):
+    """fp32 moments lose the element's own; in 8 bits its block of 128 becomes NaN, and the parameters one step later."""
+    n = 300
+    g = torch.full((n,), 0.5, device=DEV)
+    p = torch.nn.Parameter(torch.ones(n, device=DEV))
+    opt = pkg.AdamW([p], lr=1e-2, state_bits=bits)
+    g[133] = bad
+    hit, block = torch.zeros(n, dtype=torch.bool, device=DEV), torch.zeros(n, dtype=torch.bool, device=DEV)
+    hit[133], block[128:256] = True, True
+    p.grad = g
+    opt.step()
+    assert torch.equal(~torch.isfinite(p), hit)
+    m = opt.state[p]["exp_avg"].float()
+    assert torch.equal(~torch.isfinite(m), block if bits == 8 else hit)
+    p.grad = torch.full((n,), 0.5, device=DEV)
+    opt.step()
+    assert torch.equal(~torch.isfinite(p), block if bits == 8 else hit)
