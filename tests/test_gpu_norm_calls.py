@@ -1,4 +1,4 @@
-"""modulated_layer_norm and layer_norm on the GPU: many batch entries."""
+"""modulated_layer_norm and layer_norm on the GPU: many batch entries, each gradient by itself, odd addresses."""
 from __future__ import annotations
 
 import pytest
@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_layer_norm import check, reference  # noqa: E402
+from test_gpu_layer_norm import check, inputs, reference  # noqa: E402
 
 DEV = "cuda:0"
 
@@ -40,3 +40,42 @@ def test_many_entries(pkg, shape, both):
         flat = pkg.modulated_layer_norm(x.to(DEV).view(B, D), leaves[1].detach().view(B, D) if both else leaves[1].detach(),
                                         scale.to(DEV).view(B, D))
         assert torch.equal(flat, y.detach().view(B, D))
+
+
+@pytest.mark.parametrize("D", [256, 250, 2052, 5])
+def test_each_gradient_by_itself(pkg, D):
+    """The gradient of one of the leaves alone is that of all of them together (with no column sums for x's)."""
+    x, dy, e = (t.to(DEV) for t in inputs((3, 10, D), torch.bfloat16, torch.bfloat16, 5))
+    values = (x, e[:, 0:1].contiguous(), e[:, 1:2].contiguous())
+    leaves = [t.clone().requires_grad_(True) for t in values]
+    full = torch.autograd.grad(pkg.modulated_layer_norm(*leaves), leaves, dy)
+    for k in range(3):
+        one = [t.clone().requires_grad_(i == k) for i, t in enumerate(values)]
+        g, = torch.autograd.grad(pkg.modulated_layer_norm(*one), one[k], dy)
+        assert torch.equal(g, full[k]), k
+    w, b = values[1][0, 0], values[2][0, 0]
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    full = torch.autograd.grad(pkg.layer_norm(*leaves), leaves, dy)
+    for k in range(3):
+        one = [t.clone().requires_grad_(i == k) for i, t in enumerate((x, w, b))]
+        g, = torch.autograd.grad(pkg.layer_norm(*one), one[k], dy)
+        assert torch.equal(g, full[k]), k
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [256, 250, 2052, 5])
+def test_odd_addresses(pkg, D, dtype):
+    """x, dy and the weights one element behind an aligned address: the same bits, by the same loads."""
+    x, dy, e = (t.to(DEV) for t in inputs((3, 10, D), dtype, dtype, 6))
+    values = (x, e[0, 0].contiguous(), e[0, 1].contiguous())
+
+    def moved(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        buf[1:].copy_(t.reshape(-1))
+        return buf[1:].view(t.shape)
+    out = []
+    for f in (torch.clone, moved):
+        leaves = [f(t).requires_grad_(True) for t in values]
+        y = pkg.layer_norm(*leaves)
+        out.append([y.detach(), *torch.autograd.grad(y, leaves, f(dy))])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
