@@ -540,7 +540,8 @@ int hif8_attention_fwd_split(const uint16_t *q, const uint16_t *k, const uint16_
  * integer (at least -126) with max|x| <= largest * 2^e, largest = 448 (e4m3) or 57344 (e5m2), and a
  * value's code is its quotient by 2^e rounded to nearest even.  A block with an infinity or NaN has NaN
  * codes.  A matrix [rows, cols] in blocks along its rows is codes [rows, cols rounded up to 128], zeros
- * behind the last column, and scale bytes [rows, hif8_fp8_scale_row(cols)], 127 behind the last block.
+ * behind the last column (NaN in a block that has one), and scale bytes [rows, hif8_fp8_scale_row(cols)], 127 behind
+ * the last block.
  */
 #define HIF8_FP8_E4M3 0
 #define HIF8_FP8_E5M2 1
@@ -556,9 +557,11 @@ int64_t hif8_fp8_quantize_workspace_bytes(int64_t rows, int64_t cols);
 int hif8_fp8_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld, int format, int tile,
                       uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t, void *colsum,
                       int colsum_dtype, void *workspace, int64_t workspace_bytes, hif8_stream_t stream);
-/* y [M, N] = a [M, K] b [N, K]^T + bias on FP8 blocks along K, fp32 sums rounded once to y_dtype (BF16, F32 or
- * F16); bias [N] of bias_dtype or NULL.  workspace: hif8_fp8_gemm_workspace_bytes (0 for most shapes: products
- * with few output tiles and a long K are summed in K ranges).  a, b, y and workspace 16-byte aligned, scales 4. */
+/* y [M, N] = a [M, K] b [N, K]^T + bias on FP8 blocks along K.  The matrix instruction cuts the terms of 8
+ * consecutive k off towards zero 13 bits below their largest; their sums are added in fp32 and rounded once to y_dtype
+ * (BF16, F32 or F16): an F32 y is 1e-5 to 5e-5 of its norm away from the exact product.  bias [N] of bias_dtype or
+ * NULL.  workspace: hif8_fp8_gemm_workspace_bytes (0 for most shapes: products with few output tiles and a long K are
+ * summed in K ranges).  a, b, y and workspace 16-byte aligned, scales 4. */
 int64_t hif8_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int hif8_fp8_gemm(const uint8_t *a, const uint8_t *a_scales, int a_format, const uint8_t *b, const uint8_t *b_scales,
                   int b_format, const void *bias, int bias_dtype, void *y, int y_dtype, int64_t M, int64_t N, int64_t K,

@@ -168,7 +168,7 @@ def once(grad: torch.Tensor) -> None:
         raise RuntimeError("this operator can be differentiated once only (create_graph is not supported)")
 
 
-_HERE = contextlib.nullcontext()
+_CURRENT = contextlib.nullcontext()
 _FLOATS = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32, torch.float16: DTYPE_F16}
 
 
@@ -184,7 +184,7 @@ def on(device: torch.device):
     """A context in which ``device`` is the current one (launches go to the current device's context)."""
     index = device.index
     if index is None or index == torch._C._cuda_getDevice():
-        return _HERE
+        return _CURRENT
     return torch.cuda.device(device)
 
 

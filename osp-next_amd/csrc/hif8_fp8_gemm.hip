@@ -2,14 +2,18 @@
 //
 // v_mfma_scale_f32_32x32x64_f8f6f4 multiplies each 32 values of k by a power of two per row of either
 // operand.  A block's 128 values take two instructions with the same scale byte, so a product costs the
-// same as one without scales, and the accumulators hold the scaled sums in fp32 all along.  Which of the
-// 64 values of k lies in which of a lane's registers does not matter as long as both operands agree.
+// same as one without scales, and the accumulators hold the scaled sums in fp32 all along.  The instruction itself
+// cuts the terms of 8 consecutive k off towards zero, 13 bits below the largest of them: an fp32 result is 1.1e-5 to
+// 1.5e-5 of its norm away from the exact one, 4e-5 to 5e-5 where a few channels are 20 times the others (fp32 sums:
+// 1e-7).  The codes' own rounding, up to 2^-4 of a value, is far above that.  Which of the 64 values of k lies in which
+// of a lane's registers does not matter as long as both operands agree.
 //
-// What bounds it: 75600 x 13824 x 5120 takes 4.07-4.15 ms, 2.6 PFLOP/s, on random codes and 3.25 ms, 3.3 PFLOP/s, with
-// one operand zero: the card's power.  A tile of 256 x 256 takes 2.4 thousand cycles a step of 128 k (the matrix
-// instructions alone 2.0) and 14 thousand besides, for its first loads and its outputs, so that short k are slower:
-// 32760 x 8960 x 1536 440-480 us, 1.9-2.05 PFLOP/s.  (Workgroups that stay and load the next tile's first stage before
-// they write one's outputs are 1 % faster and need every register; they are not kept.)
+// What bounds it: 75600 x 13824 x 5120 takes 4.08-4.5 ms, 2.4-2.6 PFLOP/s (by the card and how warm it is), on random
+// codes and 3.25 ms, 3.3 PFLOP/s, with one operand zero: the card's power.  A tile of 256 x 256 takes 2.4 thousand
+// cycles a step of 128 k (the matrix instructions alone 2.0) and 14 thousand besides, for its first loads and its
+// outputs, so that short k are slower: 32760 x 8960 x 1536 415-480 us, 1.9-2.15 PFLOP/s.  (Workgroups that stay and load
+// the next tile's first stage before they write one's outputs are 1 % faster and need every register; they are not
+// kept.)  Outputs in fp32 instead of bf16: 75600 x 5120 x 5120 1635 us against 1550, 32760 x 1536 x 1536 95 against 80.
 #include "hif8_fp8_dev.h"
 
 namespace hif8 {
@@ -591,8 +595,9 @@ int hif8_fp8_gemm(const uint8_t *a, const uint8_t *a_scales, int a_format, const
     // 5120 22 / 24 (with two meetings a step); but with the many rows of a large grid, whose groups every eighth item covers evenly,
     // 32760 x 8960 x 1536 474 / 441, 8960 x 1536 x 32760 440 / 414.
     A.chunked = A.splits > 1 || tiles_m <= 8;
-    // 75600 x 13824 x 5120 in groups of 64 rows of tiles 4145 us, of 32 4160, of 128 4210; 8960 x 1536 x 32760 (6
-    // columns of tiles) of 32 370, of 128 427.
+    // Microseconds in groups of 16 / 32 / 64 / 128 rows of tiles.  54 columns of them, 75600 x 13824 x 5120: 4152 / 4100 /
+    // 4080 / 4144; 35, 32760 x 8960 x 1536: 421 / 415 / 415 / 429; 20, 13824 x 5120 x 32760: 2022 / 1884 / 2096 / 2095;
+    // 6, 8960 x 1536 x 32760: 361 / 358 / 423 / 422.
     A.group_shift = tiles_n >= 32 ? 6 : 5;
     A.full_groups = int(tiles_m >> A.group_shift);
     A.by_group.set(uint32_t(tiles_n << A.group_shift));

@@ -13,7 +13,7 @@ constexpr int kThreads = 256;
 
 // Codes along the rows.  16 lanes hold a block, 8 values each; a workgroup does 16 blocks at a time.
 // Unit u is block u % S of row u / S; the units past a row's last block write its padding bytes.
-// 75600 x 5120 bf16: 200 us, 5.8 TB/s.
+// 75600 x 5120 bf16: 200-212 us, 5.5-5.8 TB/s; fp32: 335 us, 5.8 TB/s.
 template <int DT, int FMT>
 __global__ __launch_bounds__(kThreads) void k_fp8_rows(const uint8_t *__restrict__ x, int64_t ld, int64_t cols,
                                                        uint32_t units, uint32_t S, uint32_t nblk,
@@ -45,7 +45,8 @@ __global__ __launch_bounds__(kThreads) void k_fp8_rows(const uint8_t *__restrict
 // out past the caches (32760 x 8960 with sums: 281 us, in fp32 and by cached stores 311).
 // bf16: 75600 x 5120 both 300-310 us, 5.0-5.1 TB/s; 32000 x 8960 with sums 235 us, 4.9 TB/s, but 32760 x 8960 276-281,
 // 4.2 TB/s (also with padded rows of the transpose; columns of tiles first 264, and 255 at 32000); 13824 x 5120 tiles
-// 45 us.
+// 45 us.  fp32 (what the self-attention hands its o projection): 75600 x 5120 both 432 us, 5.4 TB/s; 32760 x 1536 50 us,
+// 6.1 TB/s.
 template <int DT, int FMT, bool TILE>
 __global__ __launch_bounds__(kThreads, DT == HIF8_DTYPE_F32 ? 3 : 4)
 void k_fp8_both(const uint8_t *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, uint8_t *__restrict__ codes,

@@ -8,9 +8,10 @@
 // gradients are one row per group.  Statistics, sums and gradients are fp32, each output rounded once.
 //
 // Everything here is bound by memory: x is read once and y written once, and backward reads x and dy and
-// writes dx once (75600 x 5120 bf16: forward 298 us, 5.2 TB/s, backward 427 us, 5.4 TB/s).  A row stays in the registers of its threads, E values each; a workgroup walks a strip of
-// rows of one group with the group's weights in registers too, and backward keeps the strip's column sums
-// there, one partial row of each per strip, which a second kernel adds up in order.
+// writes dx once (75600 x 5120 bf16: forward 285-298 us, 5.2-5.4 TB/s, backward 430 us, 5.4 TB/s).  A row stays in
+// the registers of its threads, E values each; a workgroup walks a strip of rows of one group with the group's weights
+// in registers too, and backward keeps the strip's column sums there, one partial row of each per strip, which a
+// second kernel adds up in order.
 #include "hif8_fp8_dev.h"
 
 namespace hif8 {
@@ -362,7 +363,9 @@ __global__ __launch_bounds__(1024) void k_ln_cols(const float *__restrict__ part
 }
 
 // Rows of up to 1536 values stay in one wave, four rows a workgroup and no barrier; longer ones take 16 values a
-// thread in as many waves as they need.
+// thread in as many waves as they need.  Forward / backward in microseconds, one wave of 24 values a thread against two
+// of 16: 4681 x 1536 bf16 6.0 / 17.5 and 9.0 / 27.5, 32760 x 1536 31.6 / 53.9 and 33.5 / 63.3, 32760 x 1032 24.0 / 41.0
+// and 29.2 / 57.8, 512 x 1536 3.9 / 9.4 and 4.1 / 13.6; fp32 32760 x 1536 74.6 / 120 and 73.7 / 128.
 constexpr int kOneWave = 1536;
 template <int DT, int E, Kind KIND, bool WIDE> void launch(bool fwd, const Args &A, uint32_t groups, hipStream_t st)
 {
@@ -398,7 +401,9 @@ int value_bytes(int dt) { return dt == HIF8_DTYPE_F32 ? 4 : 2; }
 // Strips of a group.  Forward: up to 40960 waves in all (75600 rows of 5120: 302 us; 1024 workgroups 332), but not
 // less than 4 rows a wave, whose weights take as long to load as a row, unless that leaves CUs idle.  Backward:
 // about 10 waves a CU, every CU the same (5120 columns: 512 workgroups 424 us, 409 or 614 of them 487 and 503),
-// since each strip leaves two partial rows.
+// since each strip leaves two partial rows.  Backward in microseconds with 5 / 10 / 15 / 20 waves a CU: 75600 x 5120 412 /
+// 430 / 438 / 451, 512 x 5120 19 / 27 / 27 / 27, 20000 x 4096 104 / 99 / 105 / 117, 20000 x 8192 192 / 185 / 185 / 201,
+// 32760 x 2048 86 / 84 / 99 / 101, 32760 x 1536 51 / 54 / 57 / 61; fp32 20000 x 4096 198 / 214 / 211 / 216.
 int strips_of(bool fwd, int64_t groups, int64_t rows_per_group, int64_t D)
 {
     const int64_t at_once = D <= kOneWave ? 4 : 1, waves = D <= kOneWave ? 4 : (D + 1023) / 1024;

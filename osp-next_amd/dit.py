@@ -786,6 +786,7 @@ class OSPNextAttentionBlock(nn.Module):
         return n(x)
 
     def _one_pass(self, x: Tensor) -> bool:
+        """(The other routes keep the reference's sequence of fp32 operations and their roundings.)"""
         return self.quant == "fp8" and x.is_cuda and self.dim <= MAX_DIM
 
     def block_forward(self, x: Tensor, attn_mask: Optional[Tensor], cross_attn_mask: Optional[Tensor], e: Tensor,
